@@ -24,12 +24,14 @@ _X = {torch.float32: X_F32, torch.bfloat16: X_BF16}
 _OUT = {torch.float32: OUT_F32, torch.bfloat16: OUT_BF16}
 
 
-_F32, _BF16, _I32, _I64, _F8 = torch.float32, torch.bfloat16, torch.int32, torch.int64, torch.float8_e4m3fn
+_F32, _BF16, _I32, _I64 = torch.float32, torch.bfloat16, torch.int32, torch.int64
+_F8 = getattr(torch, "float8_e4m3fn", None)
 # The step's calls take about as long on the host as their kernels do: the cheapest of torch's forms that say the same (empty_strided 1.5 us,
-# empty 2.3; the raw handle of the current stream 0.1, the object 3.2), and messages made only where they are raised.
+# empty 2.3; the raw handle of the current stream 0.1, the object 3.2), and messages made only where they are raised.  The two names of torch's
+# binding are not promised by it, and a torch without CUDA has neither: the public calls stand in then.
 _memory = torch.empty_strided
-_device_now = torch._C._cuda_getDevice
-_stream_now = torch._C._cuda_getCurrentRawStream
+_device_now = getattr(torch._C, "_cuda_getDevice", None) or torch.cuda.current_device
+_stream_now = getattr(torch._C, "_cuda_getCurrentRawStream", None) or (lambda device: torch.cuda.current_stream(device).cuda_stream)
 
 
 def _here(t: torch.Tensor, name: str) -> int:
