@@ -201,7 +201,7 @@ class Rope:
 
     def __init__(self, inv_freq: torch.Tensor, pair_axis: Optional[torch.Tensor] = None, interleaved: bool = False, magnitude: float = 1.0):
         at, half = _here(inv_freq, "inv_freq"), inv_freq.numel()
-        self.inv_freq, self.pair_axis, self.interleaved, self.magnitude, self.rot_dim = inv_freq, pair_axis, interleaved, magnitude, 2 * half
+        self.inv_freq, self.pair_axis, self.interleaved, self.magnitude, self.rot_dim, self.index = inv_freq, pair_axis, interleaved, magnitude, 2 * half, at
         self.desc = capi.RopeDesc(2 * half, int(interleaved), magnitude, 0, _dense(inv_freq, "inv_freq", _F32, (half,), at),
                                   _dense(pair_axis, "pair_axis", _I32, (half,), at))
         self.ref = C.byref(self.desc)
@@ -258,6 +258,8 @@ def rope_append(q, k, v, cache: KVCache, slot, pos, rope: Rope, q_norm=None, k_n
     axes = 1 if pos.dim() == 1 else pos.shape[0]
     if pos.dtype is not _I32 or pos.get_device() != dev or pos.dim() not in (1, 2) or pos.shape[-1] < T or (T > 1 and pos.stride(-1) != 1):
         raise ValueError(f"pos: int32 [{T}] or [axes][{T}] on cuda:{dev} is needed, not {pos.dtype} {tuple(pos.shape)} on {pos.device}")
+    if rope.index != dev:
+        raise ValueError(f"the rope's frequencies are on cuda:{rope.index}, the cache is on cuda:{dev}")
     if axes != 1 and rope.pair_axis is None:
         raise ValueError("several axes need the rope's pair_axis")
     code = capi.lib().bsx_rope_append(
