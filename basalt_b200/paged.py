@@ -147,6 +147,7 @@ class PagePlan:
         self.pos, self.row = torch.empty(max_tokens, **i32), torch.empty(max_tokens, **i32)
         self.cu_new, self.seq_len = torch.empty(max_rows + 1, **i32), torch.empty(max_rows, **i32)
         self.free_count, self.status = torch.empty(1, **i32), torch.zeros(1, **i32)
+        self.index = self.status.get_device()
         self.at = tuple(t.data_ptr() for t in (self.seq_len, self.free_count, self.cu_new, self.slot, self.pos, self.row, self.status))
 
     def check_status(self) -> None:
@@ -163,6 +164,8 @@ def page_plan(seq_len, n_new, block_table, free_list, free_count, page_size: int
     n, max_pages, stride = _table(block_table, dev)
     if n > out.max_rows:
         raise ValueError(f"{n} rows: the plan's buffers hold {out.max_rows}")
+    if out.index != dev:
+        raise ValueError(f"the plan's buffers are on {out.status.device}, the rows are on cuda:{dev}")
     rows, cap = (n,), free_list.shape[0]
     code = capi.lib().bsx_page_plan(
         _dense(seq_len, "seq_len", _I32, rows, dev), _dense(n_new, "n_new", _I32, rows, dev), n, page_size, block_table.data_ptr(), stride, max_pages,

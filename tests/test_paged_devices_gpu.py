@@ -29,3 +29,19 @@ def test_a_rope_of_another_device(lib, cuda, nothing_launched):
     nothing_launched()
     with pytest.raises(ValueError, match="rope"):
         paged.rope_append(rows, rows, rows, cache, slot, pos, rope)
+
+
+@pytest.mark.parametrize("where", ["cpu", "another"])
+def test_a_plan_of_another_device(lib, cuda, nothing_launched, where):
+    ints = lambda *v: torch.tensor(v, dtype=torch.int32, device=dev)  # noqa: E731
+    good = dict(seq_len=ints(0, 0, 0), n_new=ints(1, 2, 3), block_table=torch.zeros((3, 8), dtype=torch.int32, device=dev),
+                free_list=torch.arange(30, dtype=torch.int32, device=dev), free_count=ints(30), page_size=16)
+    out = paged.PagePlan(3, 64)
+    paged.page_plan(**good, out=out)
+    if where == "cpu":
+        out = paged.PagePlan(3, 64, device="cpu")
+    else:
+        out.index = torch.cuda.current_device() + 1      # as one that was made while another device was current
+    nothing_launched()
+    with pytest.raises(ValueError, match="plan"):
+        paged.page_plan(**good, out=out)
