@@ -696,7 +696,7 @@ __global__ void __launch_bounds__(kAttnThreads, (Shape<D, NT, E4M3>::kBlocks)) p
             if (p.sinks) {
                 const float sink = p.sinks[head] * kLog2e, both = fmaxf(m, sink);
                 f *= exp2f(m - both);
-                l = l * exp2f(m - both) + exp2f(sink - both);
+                l = l * exp2f(m - both) + (sink == both ? 1.f : exp2f(sink - both));   // an infinite sink less itself is no number
                 m = both;
             }
             if (d0 == 0 && p.lse) p.lse[(int64_t) h_token * p.hq + head] = l != 0.f ? (m + log2f(l)) * kLn2 : -INFINITY;
