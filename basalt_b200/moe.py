@@ -239,26 +239,26 @@ def block_norm(y, x, post_w=None, gate=None, gate_sigmoid: bool = False, block_s
     for all ([K] or [1][K]).  Returns (h, act or None, xn or None); h has x's type (fp32 without x) and may be x itself (out=x)."""
     dev, shape, stride = _here(y, "y"), y.shape, y.stride()
     y_kind = _ROWS.get(y.dtype)
-    if y_kind is None or len(shape) != 2 or stride[1] != 1:
+    if y_kind is None or len(shape) != 2 or (stride[1] != 1 and shape[1] != 1):
         raise ValueError(f"y: fp32 or bf16 [T][K] with dense rows is needed, not {y.dtype} {tuple(shape)}")
     T, K = shape
     x_at, x_kind, x_stride, kind = None, X_F32, 0, torch.float32
     if x is not None:
         kind = x.dtype
         x_at, x_kind, x_stride = x.data_ptr(), _ROWS.get(kind), x.stride(0)
-        if x_kind is None or x.shape != shape or x.get_device() != dev or x.stride(1) != 1:
+        if x_kind is None or x.shape != shape or x.get_device() != dev or (x.stride(1) != 1 and K != 1):
             raise ValueError(f"x: fp32 or bf16 rows of y's shape {tuple(shape)} are needed, not {kind} {tuple(x.shape)} on {x.device}")
     gate_at, gate_stride = None, 0
     if gate is not None:
         rows = 1 if gate.dim() == 1 else gate.shape[0]
-        if gate.dtype is not y.dtype or gate.get_device() != dev or gate.dim() not in (1, 2) or rows not in (1, T) or gate.shape[-1] != K or gate.stride(-1) != 1:
+        if gate.dtype is not y.dtype or gate.get_device() != dev or gate.dim() not in (1, 2) or rows not in (1, T) or gate.shape[-1] != K or (gate.stride(-1) != 1 and K != 1):
             raise ValueError(f"gate: rows of y's type, [K], [1][K] or [T][K], are needed, not {gate.dtype} {tuple(gate.shape)} on {gate.device}")
         gate_at, gate_stride = gate.data_ptr(), gate.stride(0) if rows > 1 else 0
     if out is None:
         h, h_stride = _empty(shape, kind, y.device, stream), K
     else:
         h, h_stride = out, out.stride(0)
-        if h.dtype is not kind or h.shape != shape or h.get_device() != dev or h.stride(1) != 1:
+        if h.dtype is not kind or h.shape != shape or h.get_device() != dev or (h.stride(1) != 1 and K != 1):
             raise ValueError(f"out: rows of x's type {kind} and shape {tuple(shape)} are needed, not {h.dtype} {tuple(h.shape)} on {h.device}")
     a = n = a_at = n_at = None
     if pre_w is not None:

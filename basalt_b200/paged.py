@@ -95,7 +95,7 @@ class KVCache:
         if k.dtype not in (_BF16, _F8):
             raise ValueError(f"cache type {k.dtype}: bf16 or float8_e4m3fn")
         n, hk, page, d = k.shape
-        if any(t.stride()[1:] != (page * d, d, 1) for t in (k, v)):
+        if any(m != 1 and step != want for t in (k, v) for m, step, want in zip(k.shape[1:], t.stride()[1:], (page * d, d, 1))):
             raise ValueError("a page's heads, slots and values lie densely")
         f8 = k.dtype == _F8
         if (k_scale is not None) != f8 or (v_scale is not None) != f8:
@@ -129,7 +129,7 @@ class KVCache:
 
 def _table(t: torch.Tensor, device: int):
     """(rows, max_pages, stride) of a block table."""
-    if t.dtype is not _I32 or t.get_device() != device or t.dim() != 2 or t.stride(1) != 1:
+    if t.dtype is not _I32 or t.get_device() != device or t.dim() != 2 or (t.stride(1) != 1 and t.shape[1] != 1):
         raise ValueError(f"block_table: int32 [rows][max_pages] with dense rows on cuda:{device} is needed, not {t.dtype} {tuple(t.shape)} on {t.device}")
     n, m = t.shape
     return n, m, t.stride(0) if n > 1 else m
@@ -292,7 +292,7 @@ def paged_attention(q, cache: KVCache, block_table, pos, row=None, scale: Option
     t; -1: none), the last `window` of them if window > 0.  scale defaults to D ** -0.5.  Returns (out [T][heads][D], lse [T][heads] or
     None)."""
     dev, D, shape, stride = _here(q, "q"), cache.head_dim, q.shape, q.stride()
-    if q.dtype is not _BF16 or len(shape) != 3 or shape[2] != D or stride[2] != 1 or stride[1] != D or cache.index != dev:
+    if q.dtype is not _BF16 or len(shape) != 3 or shape[2] != D or stride[2] != 1 or (stride[1] != D and shape[1] != 1) or cache.index != dev:
         raise ValueError(f"q: bf16 [T][heads][{D}] with dense tokens on {cache.device} is needed, not {q.dtype} {tuple(shape)} on {q.device}")
     T, hq = shape[0], shape[1]
     n, max_pages, table_stride = _table(block_table, dev)
