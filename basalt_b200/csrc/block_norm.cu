@@ -7,9 +7,9 @@
 // four it reads and writes the same four one by one.  Sums: a thread's values, a warp's threads by butterfly, the warps in a fixed order: the
 // same for every T, stride and start.
 //
-// On a B200: 8192 rows of 7168, y bf16, x fp32, a gate for all, bf16 rows out, 705 MB: 119 us, 5.9 TB/s; 16384 of 7168, all fp32: 311 us,
-// 6.8 TB/s; one row of 2048 2.7 us; rows of 4097 bf16 values, one by one, 93 us for 4096 (30 at the rate of the others).  Rows staged
-// in shared memory by asynchronous copies, a block going from row to row: 164 us where this takes 119.
+// On a B200: 8192 rows of 7168, y bf16, x fp32, a gate for all, bf16 rows out, 705 MB: 121 us, 5.8 TB/s; 16384 of 7168, all fp32: 311 us,
+// 6.8 TB/s; one row of 2048 3.0 us; rows of 4097 bf16 values, one by one, 93 us for 4096 (30 at the rate of the others).  Rows staged
+// in shared memory by asynchronous copies, a block going from row to row: 164 us where this takes 121.
 #include "common.cuh"
 #include "pdl.cuh"
 

@@ -3,7 +3,7 @@
 //
 // Bound by HBM where there is enough to read: a key and its value come once for the G heads of their group and carry 4 G D operations, G / 2
 // a byte of bf16, G a byte of e4m3.  That keeps the tensor pipe a tenth to a fifth busy with warp-wide MMAs of 8 or 16 columns, whose operands
-// can be any lines of memory; what runs short before it is instructions (e4m3: 45 % of the issue slots), and in small calls latency.
+// can be any lines of memory (64 ragged requests 14 %, e4m3 26 %); what runs short before it is instructions, and in small calls latency.
 //
 // A warp's tile is 16 keys of one kv head.  Keys are the MMAs' rows and heads their columns, 8 a column tile (NT of them), so that a
 // group of 8 heads wastes nothing: scores S [16 keys][8 heads] = K Q^T, out O^T [D][8 heads] += V^T P^T.  Operands are read as their
@@ -31,9 +31,10 @@
 // bits do not depend on which that was; many parts are joined in two steps (131072 keys, 148 parts: 103 us in one, 56 in two).  The line's
 // running sums are made by every block itself up to 512 tokens, by a launch before beyond.
 //
-// Measured on a B200, device time in a graph, three caches in turn: 64 requests of 17 to 8191 keys, 32 / 8 heads of 128, bf16, 376 MB: 64 us,
-// 5.9 TB/s; 256 of 500 to 8000, 64 / 8, e4m3, 1.44 GB: 240 us, 6.0 TB/s; one of 131072, 16 / 2 heads of 256, bf16, 268 MB: 56 us,
-// 4.8 TB/s (400000 keys: 135 us, 6.1 TB/s); one of 1000, 32 / 4 of 128: 10.2 us, of which 5.5 are an unsplit call's.
+// Measured on a B200, device time in a graph, three caches in turn: 64 requests of 17 to 8191 keys, 32 / 8 heads of 128, bf16, 353, 420 and
+// 425 MB: 65, 74 and 76 us, 5.4 to 5.6 TB/s; 256 of 500 to 8000, 64 / 8, e4m3, 1.39, 1.44 and 1.50 GB: 255, 257 to 264 and 267 us, 5.4 to
+// 5.6 TB/s (54 % of the issue slots); one of 131072, 16 / 2 heads of 256, bf16, 268 MB: 56 us, 4.8 TB/s (400000 keys: 135 us, 6.1 TB/s); one
+// of 1000, 32 / 4 of 128: 10.2 us, of which 5.5 are an unsplit call's.
 #include "paged.cuh"
 #include "pdl.cuh"
 
@@ -878,7 +879,9 @@ Plan plan_of(const bsx_kv_cache* c, int n_q_heads, int64_t T) {
     // A kv head's sets stay together, they read the same keys.  Where there are eight sets a block and more, a block's warps have other sets
     // instead of other keys: a unit's fixed work is then one warp's for its own keys, not four warps' for a quarter each
     // (us, four warps on the keys or on the sets: 1024 requests of 64 keys, 64 / 8 heads, e4m3 91, 60; 32 / 8, bf16 84, 69; 512 of 128, e4m3
-    // 60, 49; 1000 of 700, e4m3 299, 264, bf16 451, 462; with fewer the ends of the runs cost more: 64 ragged requests, bf16 62, 75)
+    // 60, 49; 1000 of 700, e4m3 299, 264, bf16 451, 462; with fewer the ends of the runs cost more: 64 ragged requests, bf16 62, 75).
+    // The host knows T, the call's places, not how many of them hold a token: in a long window that is nearly empty the rule has the other
+    // side's cost (one token of 1000 keys, 32 / 8, bf16, in 256 places 12, in 512 25)
     r.head_warps = r.group_sets == 1 ? 1 : r.group_sets == 2 ? 2 : 4;
     if (T * r.sets >= 8ll * kMaxSms * r.blocks)
         while (r.head_warps < kWarps && r.head_warps < r.sets) r.head_warps *= 2;

@@ -8,9 +8,9 @@
 // while its first rows are under way, and asks for a row's successor before it turns the row.  pos * inv_freq is taken in 64 bits and
 // reduced to one turn there: a product in fp32 is off by 4e-3 radians at position 131072 already.
 //
-// Long calls are bound by HBM and, before it, by the instructions around two vectors a lane; short ones by latency.  On a B200: 4096 tokens,
-// 32 / 8 heads of 128, bf16, pairs as neighbours on three axes, 101 MB: 22 us, 4.6 TB/s (four values a lane 29); 64 tokens of fp32 rows with
-// norms into e4m3: 2.8 us (one block a token 6.0); one token 2.1 us.
+// Long calls are bound by HBM and, before it, by the wait for a row's loads (half of the issue slots are used) and the instructions around two
+// vectors a lane; short ones by latency.  On a B200: 4096 tokens, 32 / 8 heads of 128, bf16, pairs as neighbours on three axes, 101 MB:
+// 22 us, 4.6 TB/s (four values a lane 29); 64 tokens of fp32 rows with norms into e4m3: 2.9 us (one block a token 6.0); one token 2.3 us.
 #include "paged.cuh"
 #include "pdl.cuh"
 

@@ -523,7 +523,7 @@ BSX_API int32_t bsx_rope_append(const bsx_kv_cache* cache, const bsx_rope* rope,
  * 0 .. pos[t] of it (pos[t] < 0: none), the last `window` of them when window > 0: what bsx_page_plan gives after bsx_rope_append has
  * written the step's keys, so tokens of one request do not see those after them.  Head h reads kv head h / (n_q_heads / n_kv_heads).
  * s = scale * q.k, with softcap > 0 softcap * tanh(s / softcap); out = sum e^s v / sum e^s; sinks [n_q_heads] fp32 (or null) adds e^sink to
- * the denominator.  lse [T][n_q_heads] fp32 (or null): the logarithm of the denominator, with which parts can be joined.  A token
+ * the denominator (minus infinity: nothing; infinity: all of the weight, rows of zeros).  lse [T][n_q_heads] fp32 (or null): the logarithm of the denominator, with which parts can be joined.  A token
  * that sees no key gets zeros and lse -inf (its sink with sinks).
  * q [T][n_q_heads][head_dim] bf16, q_stride values from token to token (a multiple of 8), 16-byte aligned; out [T][n_q_heads][head_dim]
  * bf16 or fp32 (out_kind), 16-byte aligned.  n_q_heads % n_kv_heads == 0, n_q_heads <= 1024, T <= BSX_PAGED_MAX_TOKENS.
@@ -531,7 +531,11 @@ BSX_API int32_t bsx_rope_append(const bsx_kv_cache* cache, const bsx_rope* rope,
  * workspace: bsx_paged_attention_workspace_bytes (for T tokens and every smaller call over the same cache), 256-byte aligned, zeroed before
  * its first use.  Every call leaves the counters at its start at zero, whatever the call's shape; calls that may run at the same
  * time need one each.  Keys are cut into runs by the whole call, so the order of a token's fp32 sums, and with it the last bits of its row,
- * depend on the call's other tokens; the same call gives the same bits. */
+ * depend on the call's other tokens (a window of tokens checked at once and the same tokens one by one can differ there); the same call
+ * gives the same bits.
+ * T counts places, with or without a token, and decides how heads are laid on the SMs: for many short requests from T * n_kv_heads of about
+ * 2400 to 3600 on (by head_dim and heads a kv head).  A long window that is nearly empty pays for that (one token of 1000 keys, 32 / 8 heads of
+ * 128: 12 us in up to 256 places, 25 in 512, 30 in 1024): call with the places that a step needs, or keep captured steps of several lengths. */
 BSX_API size_t bsx_paged_attention_workspace_bytes(const bsx_kv_cache* cache, int32_t n_q_heads, int32_t T);
 BSX_API int32_t bsx_paged_attention(const bsx_kv_cache* cache, const void* q, int64_t q_stride, int32_t n_q_heads, int32_t T, const int32_t* block_table,
                                     int64_t table_stride, int32_t n_rows, int32_t max_pages, const int32_t* pos, const int32_t* row, float scale,
